@@ -8,8 +8,6 @@
   compact   finished sequences give their pages back, then the highest pages in use move into the lowest free ones
 """
 import math
-import os
-import sys
 
 import torch
 
@@ -257,20 +255,9 @@ def prepare(case, seed):
 
 
 # ---- the framework's calls ---------------------------------------------------------------------------------------
-_ops = None
-
-
-def _package():
-    global _ops
-    if _ops is None:
-        sys.path.insert(1, os.path.abspath("vllm-xpu-kernels_b200"))  # the folder of the package, from the repository's root
-        from vllm_xpu_kernels import ops
-        _ops = ops
-    return _ops
-
-
 def _own(s):
-    ops = _package()
+    from vllm_xpu_kernels import ops
+
     if s["op"] == "product":
         ops.fp8_block_scaled_mm(s["out"], s["a"], s["b"], s["a_scales"], s["b_scales"])
         return s["out"]
@@ -288,9 +275,7 @@ def _own(s):
             c["interleaved"], s["caches"][0], s["caches"][1], s["slots"], c["cache"], s["k_scale"], s["v_scale"],
             write_back_key=False, query_out=s["query_out"])
         return s["query_out"], s["caches"]
-    if "layers" not in s:  # the lists of all layers' caches, which a program holds from its start on
-        s["layers"] = [layer[0] for layer in s["cache"]], [layer[1] for layer in s["cache"]]
-    keys, values = s["layers"]
+    keys, values = [layer[0] for layer in s["cache"]], [layer[1] for layer in s["cache"]]
     table, lens, counts = s["table"].clone(), s["lens"].clone(), s["counts"].clone()  # the step's own copies
     if s["op"] == "fork":
         ops.fork_blocks(table, lens, counts, s["parents"], s["children"], keys, values, s["block"], s["mapping"],
