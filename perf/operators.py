@@ -255,9 +255,19 @@ def prepare(case, seed):
 
 
 # ---- the framework's calls ---------------------------------------------------------------------------------------
-def _own(s):
-    from vllm_xpu_kernels import ops
+def _ops():
+    try:
+        from vllm_xpu_kernels import ops
+    except ModuleNotFoundError:  # the package's folder lies beside this file's, wherever the program was started
+        import os
+        import sys
+        sys.path.append(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "vllm-xpu-kernels_b200"))
+        from vllm_xpu_kernels import ops
+    return ops
 
+
+def _own(s):
+    ops = _ops()
     if s["op"] == "product":
         ops.fp8_block_scaled_mm(s["out"], s["a"], s["b"], s["a_scales"], s["b_scales"])
         return s["out"]
