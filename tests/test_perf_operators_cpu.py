@@ -1,5 +1,5 @@
 """The measured operators' file: its framework calls find the package wherever the program was started, every op it calls is
-there."""
+there, and the package can be imported from the root of a checkout as it is."""
 import ast
 import os
 import subprocess
@@ -33,3 +33,8 @@ def test_the_framework_is_found(where, tmp_path):
               "ops = M._ops()\n"
               f"print(sum(callable(getattr(ops, n)) for n in {called!r}))\n", REPO if where == "root" else str(tmp_path))
     assert int(out) == len(called)
+
+
+def test_the_package_is_importable_from_the_root():
+    out = run("from vllm_xpu_kernels import ops, cabi\nprint(callable(ops.fp8_block_scaled_mm), cabi.lib().kvc_version() > 0)", REPO)
+    assert out.split() == ["True", "True"]
