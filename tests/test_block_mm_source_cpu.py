@@ -1,0 +1,33 @@
+"""What the tensor-core kernels of the block-scaled product promise about clusters and about waits that give up, and what no run
+shows: read off their source, in the order of its statements."""
+import os
+import re
+
+REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+SOURCE = os.path.join(REPO, "vllm-xpu-kernels_b200", "csrc", "fp8_block_mm_umma.cuh")
+
+
+def kernel(name):
+    """The kernel's body without comments."""
+    with open(SOURCE) as f:
+        text = re.sub(r"//[^\n]*", "", f.read())
+    at = text.index("{", text.index(")", text.index(f" {name}(")))
+    depth = 0
+    for i in range(at, len(text)):
+        depth += (text[i] == "{") - (text[i] == "}")
+        if depth == 0:
+            return text[at:i + 1]
+    raise AssertionError(name)
+
+
+def test_no_cta_is_written_before_it_has_begun():
+    """Distributed shared memory exists once every CTA of the cluster has begun: a cluster barrier comes before the first store
+    to another CTA, and each thread that arrives on the early one also waits on it, whatever its role."""
+    thin = kernel("block_mm_thin_kernel")
+    first_store = min(m.start() for m in re.finditer(r"\bst_cluster4?\(", thin))
+    arrive, wait = thin.index("cluster_begun_arrive()"), thin.rindex("cluster_begun_wait()", 0, first_store)
+    assert arrive < wait < first_store and thin.count("cluster_begun_arrive()") == 1
+    roles = re.split(r"\n  \} else (?:if \(warp >= kMmaWarp\) )?\{\n", thin[thin.index("if (warp >= kLoadWarp)"):])
+    assert len(roles) >= 3 and all(r.count("cluster_begun_wait()") == 1 for r in roles[:3])
+    wide = kernel("block_mm_wide_kernel")
+    assert wide.index("cluster_sync()") < min(wide.index("cluster_addr("), wide.index("wide_tma_load("))

@@ -91,10 +91,14 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-// Both by every thread of every CTA of the cluster; the CTAs of a cluster run at the same time.
+// By every thread of every CTA of the cluster (its CTAs are scheduled together, so the wait ends).
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The same in two halves, without ordering memory: every thread of the cluster arrives once its CTA has begun, and waits before
+// its first access to another CTA's shared memory, which is not there before that CTA has begun.
+__device__ __forceinline__ void cluster_begun_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_begun_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // The address that `local_addr` of this CTA's shared memory has in CTA `rank` of the cluster, and a store to it.
 __device__ __forceinline__ uint32_t cluster_addr(uint32_t local_addr, uint32_t rank) {
   uint32_t remote;
@@ -269,6 +273,8 @@ __global__ void __launch_bounds__(ThinCfg<TOK>::kThreads, ThinCfg<TOK>::kCtasPer
     *abort_word = 0;
     mbar_init_fence();
   }
+  __syncwarp();
+  if (p.splits > 1) cluster_begun_arrive();
   const uint32_t rank = p.splits > 1 ? cluster_rank() : 0;
   const int n_tile = blockIdx.x / p.splits;
   const int n0 = n_tile * 128, m0 = blockIdx.y * TOK;
@@ -302,6 +308,8 @@ __global__ void __launch_bounds__(ThinCfg<TOK>::kThreads, ThinCfg<TOK>::kCtasPer
     if (*abort_word)  // this warp's groups below i have been asked for
       for (int j = warp - kLoadWarp; j < i; j += kTakeTurns)
         if (j + Cfg::kStages >= i) mm_wait_limited(full + j % Cfg::kStages, (j / Cfg::kStages) & 1);
+    __syncwarp();
+    if (p.splits > 1) cluster_begun_wait();
   } else if (warp >= kMmaWarp) {
     constexpr uint32_t idesc = instr_desc_f8(128, TOK, F8 == KVC_KV_FP8_E5M2);
     Ring<Cfg::kStages, kTakeTurns> at(warp - kMmaWarp);
@@ -321,6 +329,8 @@ __global__ void __launch_bounds__(ThinCfg<TOK>::kThreads, ThinCfg<TOK>::kCtasPer
       }
       __syncwarp();
     }
+    __syncwarp();
+    if (p.splits > 1) cluster_begun_wait();
   } else {
     const int turn = (warp >> 2) % Cfg::kTurns, row = threadIdx.x & 127;
     const int col0 = (warp >> 2) / Cfg::kTurns * Cfg::kAcc;
@@ -405,6 +415,10 @@ __global__ void __launch_bounds__(ThinCfg<TOK>::kThreads, ThinCfg<TOK>::kCtasPer
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
+    // Every CTA of the cluster has begun (long ago, as a rule): its shared memory can be written.  A CTA with a short last
+    // share of the groups may come here while another one is still being launched.
+    __syncwarp();
+    if (p.splits > 1) cluster_begun_wait();
     // to the owner of the token: [rank and turn][token of the owner][row of b]
     const uint32_t part = rank * Cfg::kTurns + turn;
     if constexpr (Cfg::kTokenLanes) {
