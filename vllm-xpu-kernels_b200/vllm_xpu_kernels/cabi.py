@@ -547,9 +547,12 @@ def multi_axis_rotary_embedding_and_cache_flash(positions, query, key, value, he
         _in_dtype(cos_sin_cache), kv, _scale_ptr(k_scale, kv), _scale_ptr(v_scale, kv), _stream(stream)))
 
 
-def _cache_list(caches):
+def _cache_list(caches, ref_counts=None):
     """(array of pointers, count, pages, page stride, rows, row bytes, row stride) of dense caches [num_blocks, ...]
-    that all have the same page size; strides in bytes."""
+    that all have the same page size; strides in bytes.  The page operations take the number of pages from
+    ``ref_counts``: it must be the caches'."""
+    if caches and ref_counts is not None and caches[0].shape[0] != ref_counts.shape[0]:
+        raise RuntimeError("ref_counts must have one entry per page of the caches")
     ptrs = (ctypes.c_void_p * max(len(caches), 1))(*[c.data_ptr() for c in caches])
     if not caches:
         return ptrs, 0, 0, 0, 1, 0, 0
@@ -574,7 +577,7 @@ def copy_blocks(block_mapping, caches, stream=None) -> None:
 def fork_blocks(block_table, seq_lens, ref_counts, parents, children, caches, block_size: int, block_mapping, made,
                 stream=None) -> None:
     """``kvc_fork_blocks``: children that share their parents' full pages; ``block_mapping`` and ``made`` are outputs."""
-    ptrs, n, _, stride, rows, nbytes, row_stride = _cache_list(caches)
+    ptrs, n, _, stride, rows, nbytes, row_stride = _cache_list(caches, ref_counts)
     _check(lib().kvc_fork_blocks(
         block_table.data_ptr(), seq_lens.data_ptr(), ref_counts.data_ptr(), parents.data_ptr(), children.data_ptr(),
         parents.shape[0], block_table.shape[0], block_table.shape[1], block_table.stride(0), ref_counts.shape[0],
@@ -594,7 +597,7 @@ def free_blocks(block_table, seq_lens, ref_counts, sequences, block_size: int, s
 @_on_tensors_device
 def compact_blocks(block_table, ref_counts, caches, block_mapping, stream=None) -> None:
     """``kvc_compact_blocks``: the highest pages in use move into the lowest free ones."""
-    ptrs, n, _, stride, rows, nbytes, row_stride = _cache_list(caches)
+    ptrs, n, _, stride, rows, nbytes, row_stride = _cache_list(caches, ref_counts)
     _check(lib().kvc_compact_blocks(
         block_table.data_ptr(), ref_counts.data_ptr(), block_table.shape[0], block_table.shape[1], block_table.stride(0),
         ref_counts.shape[0], ptrs, n, stride, rows, nbytes, row_stride, block_mapping.data_ptr(), block_mapping.shape[0],
