@@ -395,17 +395,38 @@ int check_geometry(const char* op, const PageGeometry& g) {
   return KVC_OK;
 }
 
+// How the pages are cut into units: the widest access that every address and length allows, segments per row, and units per
+// pair of pages.  Refuses what does not fit a launch; fork and compact ask before their plan changes the state.
+struct PageCut {
+  int vb;
+  int64_t per_row, per_cache;
+};
+int cut_pages(const char* op, const PageGeometry& g, PageCut& cut) {
+  cut = PageCut{32, 1, 1};
+  if (g.num_caches == 0 || g.num_blocks == 0 || g.rows == 0 || g.row_bytes == 0) return KVC_OK;  // nothing to copy
+  for (; cut.vb > 1; cut.vb >>= 1) {
+    const int vb = cut.vb;
+    bool ok = g.row_bytes % vb == 0 && g.block_stride % vb == 0 && (g.rows == 1 || g.row_stride % vb == 0);
+    for (int64_t i = 0; ok && i < g.num_caches; ++i) ok = aligned(g.caches[i], vb);
+    if (ok) break;
+  }
+  cut.per_row = (g.row_bytes / cut.vb - 1) / (kCopyThreads * kCopyUnroll) + 1;
+  const int64_t caches = g.num_caches < kMaxCaches ? g.num_caches : kMaxCaches, most = ((1ll << 30) - 1) / caches;
+  if (g.rows > most || cut.per_row > most || g.rows * cut.per_row > most)
+    return fail(KVC_ERR_TOO_LARGE, std::string(op) + ": a page is too large");
+  cut.per_cache = g.rows * cut.per_row;
+  return KVC_OK;
+}
+
 // Copies the pages of `pairs` rows of `mapping` in all caches, and follows up `table_rows` rows of the table beside them.
 template <typename Rows>
 int copy_pages(const char* op, const PageGeometry& g, const int64_t* mapping, int64_t pairs, bool packed, int64_t table_rows,
                const Rows& rows, cudaStream_t st) {
   if (g.num_caches == 0 || g.num_blocks == 0 || g.rows == 0 || g.row_bytes == 0) pairs = 0;  // nothing to copy
-  int vb = 32;  // the widest access that every address and length allows
-  for (; vb > 1; vb >>= 1) {
-    bool ok = g.row_bytes % vb == 0 && g.block_stride % vb == 0 && (g.rows == 1 || g.row_stride % vb == 0);
-    for (int64_t i = 0; ok && i < g.num_caches; ++i) ok = aligned(g.caches[i], vb);
-    if (ok) break;
-  }
+  PageCut cut{1, 1, 1};
+  if (pairs > 0)
+    if (int rc = cut_pages(op, g, cut)) return rc;
+  const int vb = cut.vb;
   PageCopyParams<Rows> params{};
   params.rows = rows;
   PageCopy& p = params.c;
@@ -414,16 +435,14 @@ int copy_pages(const char* op, const PageGeometry& g, const int64_t* mapping, in
   p.row_stride = g.row_stride;
   p.row_vectors = g.row_bytes / vb;
   p.packed = packed;
-  const int64_t per_row = (p.row_vectors + kCopyThreads * kCopyUnroll - 1) / (kCopyThreads * kCopyUnroll);
   int64_t c0 = 0;
   do {
     const int64_t nc = g.num_caches - c0 < kMaxCaches ? g.num_caches - c0 : kMaxCaches;
     for (int64_t i = 0; i < nc; ++i) p.caches[i] = g.caches[c0 + i];
-    const int64_t per_pair = pairs > 0 ? nc * g.rows * per_row : 1;
-    if (per_pair >= (1ll << 30)) return fail(KVC_ERR_TOO_LARGE, std::string(op) + ": a page is too large");
+    const int64_t per_pair = pairs > 0 ? nc * cut.per_cache : 1;
     p.units_per_pair = static_cast<uint32_t>(per_pair);
-    p.segments = static_cast<uint32_t>(pairs > 0 ? g.rows * per_row : 1);
-    p.segments_per_row = static_cast<uint32_t>(pairs > 0 ? per_row : 1);
+    p.segments = static_cast<uint32_t>(cut.per_cache);
+    p.segments_per_row = static_cast<uint32_t>(cut.per_row);
     p.div_pair = FastDiv(p.units_per_pair);
     p.div_cache = FastDiv(p.segments);
     p.div_row = FastDiv(p.segments_per_row);
@@ -550,6 +569,8 @@ KVC_API int kvc_fork_blocks(int32_t* block_table, int32_t* seq_lens, int32_t* re
   p.made = made;
   p.num_forks = static_cast<int32_t>(num_forks);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  kvc::PageCut cut;
+  if (int rc = kvc::cut_pages(op, g, cut)) return rc;
   if (int rc = kvc::launch_plan(op, kvc::fork_plan_kernel, p, st)) return rc;
   return kvc::copy_pages(op, g, block_mapping, num_forks, false, num_forks, p, st);
 }
@@ -580,6 +601,7 @@ KVC_API int kvc_compact_blocks(int32_t* block_table, int32_t* ref_counts, int64_
   kvc::CompactParams p{};
   p.t = kvc::make_table(block_table, nullptr, ref_counts, num_seqs, table_width, table_stride, num_blocks, 1);
   if (int rc = kvc::check_table(op, p.t, num_seqs, table_width, 1, false)) return rc;
+  if (num_seqs > 0x3FFFFFFFll) return kvc::fail(KVC_ERR_INVALID_ARG, "compact_blocks: sizes out of range");  // a CTA per row
   if (max_moves < 0 || max_moves > 0x3FFFFFFFll)
     return kvc::fail(KVC_ERR_INVALID_ARG, "compact_blocks: bad number of moves");
   if (max_moves == 0) return KVC_OK;
@@ -588,6 +610,8 @@ KVC_API int kvc_compact_blocks(int32_t* block_table, int32_t* ref_counts, int64_
   p.mapping = block_mapping;
   p.max_moves = static_cast<int32_t>(max_moves);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  kvc::PageCut cut;
+  if (int rc = kvc::cut_pages(op, g, cut)) return rc;
   if (int rc = kvc::launch_plan(op, kvc::compact_plan_kernel, p, st)) return rc;
   return kvc::copy_pages(op, g, block_mapping, max_moves, true, table_width > 0 ? num_seqs : 0, p, st);
 }
