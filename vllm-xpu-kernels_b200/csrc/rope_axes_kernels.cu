@@ -416,7 +416,7 @@ int check_axes(AxesCall& c) {
 }
 
 // The widest item whose accesses every address, stride and length of the call allows: 16 bytes, 4 bytes, or
-// (vec_aligned false) single elements.
+// (vec_aligned false) single elements.  The table's address does not matter: its elements are gathered one by one.
 int axes_vec(const AxesCall& c, bool& vec_aligned) {
   const AxesParams& p = c.p;
   const int es = in_elem_size(c.in_dtype);
@@ -428,10 +428,6 @@ int axes_vec(const AxesCall& c, bool& vec_aligned) {
     const int64_t vb = static_cast<int64_t>(vec) * es;
     const int f = c.neox ? vec : vec / 2;
     bool ok = half % f == 0 && tail % vec == 0;
-    if (c.table_dtype == c.in_dtype) {  // the table is read f elements at a time; an fp32 table beside 16-bit tensors one
-      const int64_t fb = static_cast<int64_t>(f) * es;
-      ok = ok && aligned(p.cos_sin_cache, fb) && (half * es) % fb == 0;
-    }
     auto rows = [&](const void* base, int64_t st, int64_t sh) {
       return aligned(base, vb) && (st * es) % vb == 0 && (sh * es) % vb == 0;
     };
