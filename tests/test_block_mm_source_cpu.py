@@ -31,3 +31,13 @@ def test_no_cta_is_written_before_it_has_begun():
     assert len(roles) >= 3 and all(r.count("cluster_begun_wait()") == 1 for r in roles[:3])
     wide = kernel("block_mm_wide_kernel")
     assert wide.index("cluster_sync()") < min(wide.index("cluster_addr("), wide.index("wide_tma_load("))
+
+
+def test_lanes_leave_a_loop_together():
+    """A warp that breaks out of its loop when a wait gives up does so as a whole: elect.sync and the barriers behind the loop
+    need all of its lanes."""
+    for name in ("block_mm_thin_kernel", "block_mm_wide_kernel"):
+        body = kernel(name)
+        assert re.search(r"\bmm_wait\(", body)
+        for m in re.finditer(r"\bmbar_wait_bounded\(", body):  # these are statements of their own: the warp goes on
+            assert re.search(r"[;{})]\s*$", body[:m.start()]) and not re.search(r"if \(!?$", body[:m.start()])

@@ -35,6 +35,10 @@ __device__ __forceinline__ void mm_tma_load(uint32_t dst, const CUtensorMap* map
 __device__ __forceinline__ void mm_expect_tx(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(umma::smem_addr(bar)), "r"(bytes) : "memory");
 }
+// A wait by a whole warp whose lanes then go on together, whatever each of them saw.
+__device__ __forceinline__ bool mm_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_word) {
+  return __all_sync(0xFFFFFFFFu, umma::mbar_wait_bounded(bar, parity, abort_word));
+}
 // A wait that ignores the abort word: lets copies in flight land before the CTA ends.
 __device__ __forceinline__ void mm_wait_limited(uint64_t* bar, uint32_t parity) {
   for (uint32_t i = 0; i < umma::kMaxTries; ++i)
@@ -296,7 +300,7 @@ __global__ void __launch_bounds__(ThinCfg<TOK>::kThreads, ThinCfg<TOK>::kCtasPer
     int i = warp - kLoadWarp;
     for (; i < count; i += kTakeTurns, at.advance()) {
       // a slot is free from the start (the round "before" the first counts as finished)
-      if (!mbar_wait_bounded(empty + at.slot, at.parity ^ 1, abort_word)) break;
+      if (!mm_wait(empty + at.slot, at.parity ^ 1, abort_word)) break;
       if (elect_one()) {
         mm_expect_tx(full + at.slot, Cfg::kStageBytes);
         const uint32_t dst = smem_addr(smem + at.slot * Cfg::kStageBytes);
@@ -315,8 +319,8 @@ __global__ void __launch_bounds__(ThinCfg<TOK>::kThreads, ThinCfg<TOK>::kCtasPer
     Ring<Cfg::kStages, kTakeTurns> at(warp - kMmaWarp);
     Ring<Cfg::kBuffers, kTakeTurns> buf(warp - kMmaWarp);
     for (int i = warp - kMmaWarp; i < count; i += kTakeTurns, at.advance(), buf.advance()) {
-      if (!mbar_wait_bounded(taken + buf.slot, buf.parity ^ 1, abort_word)) break;
-      if (!mbar_wait_bounded(full + at.slot, at.parity, abort_word)) break;
+      if (!mm_wait(taken + buf.slot, buf.parity ^ 1, abort_word)) break;
+      if (!mm_wait(full + at.slot, at.parity, abort_word)) break;
       fence_after_thread_sync();
       if (elect_one()) {
         const uint32_t base = smem_addr(smem + at.slot * Cfg::kStageBytes);
@@ -653,7 +657,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         wide_tile(p, tile, mt, nt);
         const int m0 = mt * 256 + rank * 128, n0 = nt * 256 + rank * 128;
         for (int g = 0; g < p.groups; ++g, ++issued, at.advance()) {
-          ok = mbar_wait_bounded(empty + at.slot, at.parity ^ 1, abort_word);
+          ok = mm_wait(empty + at.slot, at.parity ^ 1, abort_word);
           if (!ok) break;
           if (elect_one()) {
             if (rank == 0) mm_expect_tx(full + at.slot, 2 * Cfg::kStageBytes);
@@ -680,7 +684,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         const float* sb0 = p.b_scales + min(nt * 2, last) * p.bs_stride_n;
         const float* sb1 = p.b_scales + min(nt * 2 + 1, last) * p.bs_stride_n;
         for (int g = 0; g < p.groups; g += Cfg::kScaleGroups, at.advance()) {
-          ok = mbar_wait_bounded(used + at.slot, at.parity ^ 1, abort_word);
+          ok = mm_wait(used + at.slot, at.parity ^ 1, abort_word);
           if (!ok) break;
           const int m = mt * 256 + static_cast<int>(rank) * 128 + lane;
           float vb[2][4];
@@ -718,8 +722,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       const int mine = pair < tiles ? (tiles - 1 - pair) / pairs + 1 : 0;  // tiles of this pair
       const int64_t steps = static_cast<int64_t>(mine) * p.groups;
       for (int64_t it = me; it < steps; it += 2, at.advance(), parity ^= 1) {
-        if (!mbar_wait_bounded(taken + me, parity ^ 1, abort_word)) break;
-        if (!mbar_wait_bounded(full + at.slot, at.parity, abort_word)) break;
+        if (!mm_wait(taken + me, parity ^ 1, abort_word)) break;
+        if (!mm_wait(full + at.slot, at.parity, abort_word)) break;
         fence_after_thread_sync();
         if (elect_one()) {
           const uint32_t base = smem_addr(smem + at.slot * Cfg::kStageBytes);
