@@ -33,6 +33,22 @@ def test_no_cta_is_written_before_it_has_begun():
     assert wide.index("cluster_sync()") < min(wide.index("cluster_addr("), wide.index("wide_tma_load("))
 
 
+def test_nothing_is_in_flight_when_memory_is_given_back():
+    """A wait can give up in any warp until the last barrier, so only behind it is it known whether copies and MMAs may still be
+    under way; they are waited for there, before the tensor memory is freed and the CTA ends."""
+    for name, barrier, free in (("block_mm_thin_kernel", "__syncthreads()", "tmem_dealloc("),
+                                ("block_mm_wide_kernel", "cluster_sync()", "tmem_dealloc_pair(")):
+        body = kernel(name)
+        drain, end = body.rindex("if (*abort_word) {"), body.index(free)
+        # behind the last wait that can give up and a barrier of everyone, and with another such barrier before the memory goes
+        last_wait = max(m.end() for m in re.finditer(r"\b(mm_wait|mbar_wait_bounded)\(", body))
+        assert last_wait < body.rindex(barrier, 0, drain) < drain < body.rindex(barrier, 0, end) < end
+        drains = [m.start() for m in re.finditer(r"\bmm_wait_limited\(", body)]
+        assert len(drains) == 2 and all(drain < d < end for d in drains)
+        commit = re.search(r"mma_commit(_pair)?\(drained\)", body)
+        assert drain < commit.start() < drains[1]
+
+
 def test_lanes_leave_a_loop_together():
     """A warp that breaks out of its loop when a wait gives up does so as a whole: elect.sync and the barriers behind the loop
     need all of its lanes."""

@@ -6,8 +6,9 @@
 // the next groups.  The scales thus never meet the operands and cost one fused multiply-add per element and group.
 //
 // Operands come in by TMA (128-byte swizzle, plain loads): columns past K and rows past the matrix read as zeros.
-// Every wait on an mbarrier is bounded; a wait that gives up sets the CTA's abort word, the CTA runs to its end, waits
-// (bounded) for its copies in flight, frees its tensor memory and raises g_block_mm_status.
+// Every wait on an mbarrier is bounded; a wait that gives up sets the CTA's abort word.  The CTA runs to its end and, once none
+// of its threads can wait any more, waits (bounded) for its copies and MMAs in flight, frees its tensor memory and raises
+// g_block_mm_status.
 #pragma once
 
 #include <cuda.h>
@@ -39,7 +40,7 @@ __device__ __forceinline__ void mm_expect_tx(uint64_t* bar, uint32_t bytes) {
 __device__ __forceinline__ bool mm_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_word) {
   return __all_sync(0xFFFFFFFFu, umma::mbar_wait_bounded(bar, parity, abort_word));
 }
-// A wait that ignores the abort word: lets copies in flight land before the CTA ends.
+// A wait that ignores the abort word: lets what is in flight land before the CTA ends.
 __device__ __forceinline__ void mm_wait_limited(uint64_t* bar, uint32_t parity) {
   for (uint32_t i = 0; i < umma::kMaxTries; ++i)
     if (umma::mbar_try_wait(bar, parity, umma::kTryNs)) return;
@@ -197,7 +198,7 @@ struct ThinCfg {
   static constexpr int kSumRow = kTokenLanes ? 132 : 128;
   static constexpr int kSumBytes = kTurns * (TOK + 7) * kSumRow * 4;  // splits * ceil(TOK / splits) rows
   static constexpr int kOffBar = kOffSums + kSumBytes;
-  static constexpr int kBars = 2 * kStages + 2 * kBuffers;
+  static constexpr int kBars = 2 * kStages + 2 * kBuffers + 1;
   static constexpr int kUsed = kOffBar + kBars * 8 + 16;
   // So much that kCtasPerSm CTAs fit an SM and no more: their tensor memory is then always there (CTAs of two clusters
   // could otherwise wait for each other's).
@@ -258,6 +259,7 @@ __global__ void __launch_bounds__(ThinCfg<TOK>::kThreads, ThinCfg<TOK>::kCtasPer
   uint64_t* empty = full + Cfg::kStages;
   uint64_t* ready = empty + Cfg::kStages;       // a group's products are in tensor memory
   uint64_t* taken = ready + Cfg::kBuffers;      // and have been read
+  uint64_t* drained = taken + Cfg::kBuffers;    // after a wait that gave up: no MMA is in flight
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::kBars);
   volatile uint32_t* abort_word = tmem_slot + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -274,6 +276,7 @@ __global__ void __launch_bounds__(ThinCfg<TOK>::kThreads, ThinCfg<TOK>::kCtasPer
       mbar_init(ready + i, 1);
       mbar_init(taken + i, 4 * Cfg::kSplit);
     }
+    mbar_init(drained, Cfg::kIssuers);
     *abort_word = 0;
     mbar_init_fence();
   }
@@ -294,24 +297,21 @@ __global__ void __launch_bounds__(ThinCfg<TOK>::kThreads, ThinCfg<TOK>::kCtasPer
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = *tmem_slot;
   float* sums = reinterpret_cast<float*>(smem + Cfg::kOffSums);
+  int asked = warp - kLoadWarp;  // a loading warp has asked for its groups below this one
 
   if (warp >= kLoadWarp) {
     Ring<Cfg::kStages, kTakeTurns> at(warp - kLoadWarp);
-    int i = warp - kLoadWarp;
-    for (; i < count; i += kTakeTurns, at.advance()) {
+    for (; asked < count; asked += kTakeTurns, at.advance()) {
       // a slot is free from the start (the round "before" the first counts as finished)
       if (!mm_wait(empty + at.slot, at.parity ^ 1, abort_word)) break;
       if (elect_one()) {
         mm_expect_tx(full + at.slot, Cfg::kStageBytes);
         const uint32_t dst = smem_addr(smem + at.slot * Cfg::kStageBytes);
-        mm_tma_load(dst, &maps.b, full + at.slot, (g0 + i) * 128, n0);
-        mm_tma_load(dst + Cfg::kTileB, &maps.a, full + at.slot, (g0 + i) * 128, m0);
+        mm_tma_load(dst, &maps.b, full + at.slot, (g0 + asked) * 128, n0);
+        mm_tma_load(dst + Cfg::kTileB, &maps.a, full + at.slot, (g0 + asked) * 128, m0);
       }
       __syncwarp();
     }
-    if (*abort_word)  // this warp's groups below i have been asked for
-      for (int j = warp - kLoadWarp; j < i; j += kTakeTurns)
-        if (j + Cfg::kStages >= i) mm_wait_limited(full + j % Cfg::kStages, (j / Cfg::kStages) & 1);
     __syncwarp();
     if (p.splits > 1) cluster_begun_wait();
   } else if (warp >= kMmaWarp) {
@@ -535,6 +535,19 @@ __global__ void __launch_bounds__(ThinCfg<TOK>::kThreads, ThinCfg<TOK>::kCtasPer
   fence_before_thread_sync();
   __syncthreads();
   fence_after_thread_sync();
+  if (*abort_word) {  // final by now
+    if (warp >= kLoadWarp) {
+      for (int j = warp - kLoadWarp; j < asked; j += kTakeTurns)
+        if (j + Cfg::kStages >= asked) mm_wait_limited(full + j % Cfg::kStages, (j / Cfg::kStages) & 1);
+    } else if (warp >= kMmaWarp) {
+      if (elect_one()) mma_commit(drained);
+      mm_wait_limited(drained, 0);
+    }
+    __syncwarp();
+    fence_before_thread_sync();
+    __syncthreads();
+    fence_after_thread_sync();
+  }
   if (warp == kMmaWarp) tmem_dealloc(tmem, Cfg::kCols);
   if (threadIdx.x == 0 && *abort_word) atomicMax(&g_block_mm_status, 1);
 }
@@ -560,7 +573,7 @@ struct WideCfg {
   static constexpr int kOffScales = kStages * kStageBytes;        // [slot][column half][row][group]
   static constexpr int kOffTurn = kOffScales + kScaleSlots * 256 * kScaleGroups * 4;
   static constexpr int kOffBar = kOffTurn + 8 * 32 * 17 * 4;      // a 32 x 16 block of results per epilogue warp
-  static constexpr int kBars = 2 * kStages + 4 + 2 * kScaleSlots;
+  static constexpr int kBars = 2 * kStages + 4 + 2 * kScaleSlots + 1;
   static constexpr int kSmem = kOffBar + kBars * 8 + 16 + 1024;
   static_assert(kSmem <= 232448 && 2 * (kSmem + 1024) > 233472, "one CTA per SM");
 };
@@ -611,8 +624,10 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   uint64_t* taken = ready + 2;                     // the even CTA's: and have been read by both CTAs
   uint64_t* scaled = taken + 2;                    // a slot's scales are there
   uint64_t* used = scaled + Cfg::kScaleSlots;      // and have been read
+  uint64_t* drained = used + Cfg::kScaleSlots;     // after a wait that gave up: no MMA of the pair is in flight
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::kBars);
   volatile uint32_t* abort_word = tmem_slot + 1;
+  volatile uint32_t* peer_asked = tmem_slot + 2;   // the even CTA's: groups that the odd one has asked for
   float4* scales = reinterpret_cast<float4*>(smem + Cfg::kOffScales);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
@@ -632,6 +647,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       mbar_init(scaled + i, 1);
       mbar_init(used + i, 8);
     }
+    mbar_init(drained, 2);
     *abort_word = 0;
     mbar_init_fence();
   }
@@ -645,18 +661,18 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   const uint32_t tmem = *tmem_slot;
   const int tiles = p.m_tiles * p.n_tiles;
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  uint32_t asked = 0;  // groups that the loading warp has asked for
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideOtherRegs));
     if (warp == 10) {
       Ring<Cfg::kStages> at;
-      uint32_t issued = 0;
       bool ok = true;
       for (int tile = pair; ok && tile < tiles; tile += pairs) {
         int mt, nt;
         wide_tile(p, tile, mt, nt);
         const int m0 = mt * 256 + rank * 128, n0 = nt * 256 + rank * 128;
-        for (int g = 0; g < p.groups; ++g, ++issued, at.advance()) {
+        for (int g = 0; g < p.groups; ++g, ++asked, at.advance()) {
           ok = mm_wait(empty + at.slot, at.parity ^ 1, abort_word);
           if (!ok) break;
           if (elect_one()) {
@@ -669,10 +685,6 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           __syncwarp();
         }
       }
-      // both CTAs' copies count on the even CTA's barriers, and neither CTA ends before the other (see the end)
-      if (*abort_word && rank == 0)
-        for (uint32_t i = issued > Cfg::kStages ? issued - Cfg::kStages : 0; i < issued; ++i)
-          mm_wait_limited(full + i % Cfg::kStages, (i / Cfg::kStages) & 1);
     } else if (warp == 11) {
       Ring<Cfg::kScaleSlots> at;
       bool ok = true;
@@ -866,9 +878,27 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     }
   }
   __syncwarp();
+  // the CTAs of a pair give up together: copies and MMAs of either touch barriers or memory of the other
+  if (*abort_word) st_cluster(cluster_addr(smem_addr(tmem_slot + 1), rank ^ 1), 1);
+  if (rank == 1 && warp == 10 && lane == 0) st_cluster(cluster_addr(smem_addr(tmem_slot + 2), 0), asked);
+  __syncwarp();
   fence_before_thread_sync();
   cluster_sync();  // the even CTA's MMAs read the odd one's shared memory, and barriers are signalled across
   fence_after_thread_sync();
+  if (*abort_word) {  // final by now, and the same in both
+    if (rank == 0 && warp == 10) {  // both CTAs' copies count on the even one's barriers
+      const uint32_t end = max(asked, *peer_asked);
+      for (uint32_t i = end > Cfg::kStages ? end - Cfg::kStages : 0; i < end; ++i)
+        mm_wait_limited(full + i % Cfg::kStages, (i / Cfg::kStages) & 1);
+    } else if (warp == 8 || warp == 9) {
+      if (rank == 0 && elect_one()) mma_commit_pair(drained);
+      mm_wait_limited(drained, 0);
+    }
+    __syncwarp();
+    fence_before_thread_sync();
+    cluster_sync();
+    fence_after_thread_sync();
+  }
   if (warp == 8) tmem_dealloc_pair(tmem, 512);
   if (threadIdx.x == 0 && *abort_word) atomicMax(&g_block_mm_status, 1);
 }
