@@ -284,8 +284,8 @@ KVC_API int kvc_dynamic_per_token_group_scaled_fp8_quant(void* out, const void* 
  * 16 bytes.  No workspace, no atomics: the same inputs give the same bits.
  *
  * kvc_fp8_block_scaled_mm_device_status waits for the device's earlier work and reads the tensor-core kernels' status
- * word: 0 = fine, 1 = a bounded wait on an mbarrier gave up (results of that call are then undefined; the kernel still
- * ran to its end and freed its tensor memory).  The word stays raised until
+ * word: 0 = fine, 1 = a bounded wait on an mbarrier gave up (results that the call could not compute are then NaN; the
+ * kernel still ran to its end and freed its tensor memory).  The word stays raised until
  * kvc_fp8_block_scaled_mm_clear_device_status (which also waits for the device's earlier work) puts it back to 0.
  */
 KVC_API int kvc_fp8_block_scaled_mm(void* out, const void* a, const void* b, const float* a_scales,

@@ -57,3 +57,21 @@ def test_lanes_leave_a_loop_together():
         assert re.search(r"\bmm_wait\(", body)
         for m in re.finditer(r"\bmbar_wait_bounded\(", body):  # these are statements of their own: the warp goes on
             assert re.search(r"[;{})]\s*$", body[:m.start()]) and not re.search(r"if \(!?$", body[:m.start()])
+
+
+def test_results_that_could_not_be_computed_are_nan():
+    """Whoever writes results looks at the abort word first, behind the last wait that they depend on: in the kernel for few rows
+    after every CTA of the cluster has told the others, in the other one once per tile."""
+    thin = kernel("block_mm_thin_kernel")
+    tell = thin.index("st_cluster(cluster_addr(smem_addr(tmem_slot + 1), r), 1)")
+    look = thin.index("const bool lost = *abort_word")
+    assert tell < thin.index("cluster_sync()", tell) < look
+    last_wait = max(m.end() for m in re.finditer(r"\b(mm_wait|mbar_wait_bounded)\(", thin))
+    assert last_wait < tell
+    stores = [m.group(0) for m in re.finditer(r"from_f32<Tout>\([^;]*;|store_words<Tout, 32>\([^;]*;", thin[look:])]
+    assert len(stores) == 2 and all("lost ? " in s for s in stores)
+    wide = kernel("block_mm_wide_kernel")
+    look = wide.index("if (*abort_word) {")
+    epilogue = wide.index("setmaxnreg.inc")
+    waits = [m.end() for m in re.finditer(r"\b(mm_wait|mbar_wait_bounded)\(", wide[epilogue:])]
+    assert epilogue + max(waits) < look < wide.index("store_chunk(") < wide.index("st_if(")

@@ -8,7 +8,7 @@
 // Operands come in by TMA (128-byte swizzle, plain loads): columns past K and rows past the matrix read as zeros.
 // Every wait on an mbarrier is bounded; a wait that gives up sets the CTA's abort word.  The CTA runs to its end and, once none
 // of its threads can wait any more, waits (bounded) for its copies and MMAs in flight, frees its tensor memory and raises
-// g_block_mm_status.
+// g_block_mm_status.  Results that it could not compute are written as NaN: nobody takes them for a product.
 #pragma once
 
 #include <cuda.h>
@@ -476,10 +476,18 @@ __global__ void __launch_bounds__(ThinCfg<TOK>::kThreads, ThinCfg<TOK>::kCtasPer
     }
   }
   __syncwarp();
-  if (p.splits > 1) cluster_sync();
-  else __syncthreads();
+  if (p.splits > 1) {
+    if (*abort_word)  // every CTA of the cluster lacks a part then
+      for (int r = 0; r < p.splits; ++r) st_cluster(cluster_addr(smem_addr(tmem_slot + 1), r), 1);
+    __syncwarp();
+    cluster_sync();
+  } else {
+    __syncthreads();
+  }
   if (warp < Cfg::kEpilogueWarps) {
     const int parts = Cfg::kTurns * p.splits;
+    const bool lost = *abort_word;
+    const float nan = __int_as_float(0x7FFFFFFF);
     if (p.wide_stores) {
       // a thread adds up eight neighbouring columns of one token
       const int c = (threadIdx.x & 15) * 8;
@@ -500,7 +508,7 @@ __global__ void __launch_bounds__(ThinCfg<TOK>::kThreads, ThinCfg<TOK>::kCtasPer
         Tout* out = static_cast<Tout*>(p.out) + m * p.out_stride + n0 + c;
         Chunk<8 * (int)sizeof(Tout)> piece;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) reinterpret_cast<Tout*>(piece.b)[j] = from_f32<Tout>(sum[j]);
+        for (int j = 0; j < 8; ++j) reinterpret_cast<Tout*>(piece.b)[j] = from_f32<Tout>(lost ? nan : sum[j]);
         if (left >= 8) {
           store_chunk(out, piece, false);
         } else {
@@ -526,7 +534,7 @@ __global__ void __launch_bounds__(ThinCfg<TOK>::kThreads, ThinCfg<TOK>::kCtasPer
             x += from[0];
             if constexpr (kPer == 2) y += from[kPer - 1];
           }
-          store_words<Tout, 32>(result_word<Tout>(x, y), lane, out + c, p.n - n0 - c);
+          store_words<Tout, 32>(lost ? result_word<Tout>(nan, nan) : result_word<Tout>(x, y), lane, out + c, p.n - n0 - c);
         }
       }
     }
@@ -793,6 +801,11 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           if (c + 32 < 128) tmem_ld_wait();
         }
         if (k == Cfg::kScaleGroups - 1 || g + 1 == p.groups) at.advance();
+      }
+      if (*abort_word) {  // set before a wait of this tile or an earlier one returned without its event
+        const uint32_t nan = 0x7FFFFFFFu;
+#pragma unroll
+        for (int j = 0; j < 64; ++j) acc[j] = pack2(nan, nan);
       }
       int mt, nt;
       wide_tile(p, tile, mt, nt);
