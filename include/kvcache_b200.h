@@ -287,6 +287,9 @@ KVC_API int kvc_dynamic_per_token_group_scaled_fp8_quant(void* out, const void* 
  * word: 0 = fine, 1 = a bounded wait on an mbarrier gave up (results that the call could not compute are then NaN; the
  * kernel still ran to its end and freed its tensor memory).  The word stays raised until
  * kvc_fp8_block_scaled_mm_clear_device_status (which also waits for the device's earlier work) puts it back to 0.
+ *
+ * kvc_fp8_block_scaled_mm_selftest_gives_up runs that path on purpose: one CTA waits for an arrival that nothing makes, for
+ * `tries` tries of about 20 us each (1..5000), gives up, drains, frees its tensor memory and raises the word.
  */
 KVC_API int kvc_fp8_block_scaled_mm(void* out, const void* a, const void* b, const float* a_scales,
                                     const float* b_scales, int64_t m, int64_t n, int64_t k, int64_t out_stride,
@@ -296,6 +299,7 @@ KVC_API int kvc_fp8_block_scaled_mm(void* out, const void* a, const void* b, con
 
 KVC_API int kvc_fp8_block_scaled_mm_device_status(int* status);
 KVC_API int kvc_fp8_block_scaled_mm_clear_device_status(void);
+KVC_API int kvc_fp8_block_scaled_mm_selftest_gives_up(int64_t tries, void* stream);
 
 /*
  * Rotary position embedding, in place.  Replaces rotary_embedding of the reference: host launcher

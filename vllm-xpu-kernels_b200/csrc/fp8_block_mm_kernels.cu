@@ -328,6 +328,18 @@ KVC_API int kvc_fp8_block_scaled_mm_clear_device_status(void) {
   return KVC_OK;
 }
 
+KVC_API int kvc_fp8_block_scaled_mm_selftest_gives_up(int64_t tries, void* stream) {
+  if (tries < 1 || tries > 5000)
+    return kvc::fail(KVC_ERR_INVALID_ARG,
+                     "fp8_block_scaled_mm_selftest_gives_up: tries must be within 1..5000 (about 20 us each)");
+  kvc::block_mm_gives_up_kernel<<<1, 128, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<uint32_t>(tries));
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess)
+    return kvc::fail(KVC_ERR_CUDA,
+                     std::string("fp8_block_scaled_mm_selftest_gives_up launch failed: ") + cudaGetErrorString(e));
+  return KVC_OK;
+}
+
 KVC_API int kvc_fp8_block_scaled_mm(void* out, const void* a, const void* b, const float* a_scales,
                                     const float* b_scales, int64_t m, int64_t n, int64_t k, int64_t out_stride,
                                     int64_t a_stride, int64_t b_stride, int64_t a_scale_stride_m,

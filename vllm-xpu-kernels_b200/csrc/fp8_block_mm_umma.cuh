@@ -37,8 +37,9 @@ __device__ __forceinline__ void mm_expect_tx(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(umma::smem_addr(bar)), "r"(bytes) : "memory");
 }
 // A wait by a whole warp whose lanes then go on together, whatever each of them saw.
-__device__ __forceinline__ bool mm_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_word) {
-  return __all_sync(0xFFFFFFFFu, umma::mbar_wait_bounded(bar, parity, abort_word));
+__device__ __forceinline__ bool mm_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_word,
+                                        uint32_t max_tries = umma::kMaxTries) {
+  return __all_sync(0xFFFFFFFFu, umma::mbar_wait_bounded(bar, parity, abort_word, max_tries));
 }
 // A wait that ignores the abort word: lets what is in flight land before the CTA ends.
 __device__ __forceinline__ void mm_wait_limited(uint64_t* bar, uint32_t parity) {
@@ -913,6 +914,44 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     fence_after_thread_sync();
   }
   if (warp == 8) tmem_dealloc_pair(tmem, 512);
+  if (threadIdx.x == 0 && *abort_word) atomicMax(&g_block_mm_status, 1);
+}
+
+// Self-test of what a CTA does when a wait gives up: one warp waits, with a limit of `tries` tries (about 20 us each), for an
+// arrival that nothing makes; the CTA then drains, frees its tensor memory and raises the status word as the kernels above do.
+__global__ void __launch_bounds__(128) block_mm_gives_up_kernel(uint32_t tries) {
+  using namespace umma;
+  __shared__ __align__(8) uint64_t bar, drained;
+  __shared__ uint32_t tmem_slot, abort_slot;
+  volatile uint32_t* abort_word = &abort_slot;
+  const int warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    mbar_init(&bar, 1);
+    mbar_init(&drained, 1);
+    *abort_word = 0;
+    mbar_init_fence();
+  }
+  __syncwarp();
+  if (warp == 0) tmem_alloc(&tmem_slot, 32);
+  fence_before_thread_sync();
+  __syncthreads();
+  fence_after_thread_sync();
+  const uint32_t tmem = tmem_slot;
+  if (warp == 1) mm_wait(&bar, 0, abort_word, tries);
+  fence_before_thread_sync();
+  __syncthreads();
+  fence_after_thread_sync();
+  if (*abort_word) {
+    if (warp == 2) {
+      if (elect_one()) mma_commit(&drained);
+      mm_wait_limited(&drained, 0);
+    }
+    __syncwarp();
+    fence_before_thread_sync();
+    __syncthreads();
+    fence_after_thread_sync();
+  }
+  if (warp == 0) tmem_dealloc(tmem, 32);
   if (threadIdx.x == 0 && *abort_word) atomicMax(&g_block_mm_status, 1);
 }
 

@@ -49,6 +49,7 @@ SYMBOLS = (
     "kvc_fp8_block_scaled_mm",
     "kvc_fp8_block_scaled_mm_device_status",
     "kvc_fp8_block_scaled_mm_clear_device_status",
+    "kvc_fp8_block_scaled_mm_selftest_gives_up",
     "kvc_multi_axis_rotary_embedding",
     "kvc_multi_axis_rotary_embedding_and_cache_flash",
     "kvc_copy_blocks",
@@ -125,6 +126,8 @@ def lib() -> ctypes.CDLL:
         L.kvc_fp8_block_scaled_mm_device_status.argtypes = [ctypes.POINTER(ci)]
         L.kvc_fp8_block_scaled_mm_clear_device_status.restype = ci
         L.kvc_fp8_block_scaled_mm_clear_device_status.argtypes = []
+        L.kvc_fp8_block_scaled_mm_selftest_gives_up.restype = ci
+        L.kvc_fp8_block_scaled_mm_selftest_gives_up.argtypes = [i64, vp]
         L.kvc_multi_axis_rotary_embedding.restype = ci
         L.kvc_multi_axis_rotary_embedding.argtypes = [vp] * 7 + [i64] * 16 + [ci] * 4 + [vp]
         L.kvc_multi_axis_rotary_embedding_and_cache_flash.restype = ci
@@ -505,6 +508,12 @@ def fp8_block_scaled_mm_device_status() -> int:
 def fp8_block_scaled_mm_clear_device_status() -> None:
     """``kvc_fp8_block_scaled_mm_clear_device_status``: waits for the device and puts the status word back to 0."""
     _check(lib().kvc_fp8_block_scaled_mm_clear_device_status())
+
+
+def fp8_block_scaled_mm_selftest_gives_up(tries: int = 50, stream=None) -> None:
+    """``kvc_fp8_block_scaled_mm_selftest_gives_up``: launches the one-CTA kernel whose bounded wait runs out; afterwards
+    ``fp8_block_scaled_mm_device_status()`` is 1 until it is cleared."""
+    _check(lib().kvc_fp8_block_scaled_mm_selftest_gives_up(int(tries), _stream(stream)))
 
 
 def _sections(axis_sections):
