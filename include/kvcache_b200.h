@@ -283,6 +283,9 @@ KVC_API int kvc_dynamic_per_token_group_scaled_fp8_quant(void* out, const void* 
  * rounded once.  Any m, n, k and strides; the tensor cores are used where a, b and their row strides are multiples of
  * 16 bytes.  No workspace, no atomics: the same inputs give the same bits.
  *
+ * kvc_fp8_block_scaled_mm_plan tells, without a GPU, which kernel such a call uses on the tensor cores: rows of a per tile (16,
+ * 32, 64 or 128, with 128 rows of b; 256: pairs of CTAs on 256 x 256 tiles) and the CTAs that divide the groups of a tile.
+ *
  * kvc_fp8_block_scaled_mm_device_status waits for the device's earlier work and reads the tensor-core kernels' status
  * word: 0 = fine, 1 = a bounded wait on an mbarrier gave up (results that the call could not compute are then NaN; the
  * kernel still ran to its end and freed its tensor memory).  The word stays raised until
@@ -297,6 +300,7 @@ KVC_API int kvc_fp8_block_scaled_mm(void* out, const void* a, const void* b, con
                                     int64_t a_scale_stride_g, int64_t b_scale_stride_n, int64_t b_scale_stride_g,
                                     int out_dtype, int fp8_dtype, void* stream);
 
+KVC_API int kvc_fp8_block_scaled_mm_plan(int64_t m, int64_t n, int64_t k, int32_t* tile_tokens, int32_t* splits);
 KVC_API int kvc_fp8_block_scaled_mm_device_status(int* status);
 KVC_API int kvc_fp8_block_scaled_mm_clear_device_status(void);
 KVC_API int kvc_fp8_block_scaled_mm_selftest_gives_up(int64_t tries, void* stream);

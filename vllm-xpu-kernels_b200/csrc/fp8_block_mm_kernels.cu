@@ -223,6 +223,12 @@ MmPlan plan_mm(const BlockMmParams& p) {
   return best;
 }
 
+// The CTAs of a cluster that have groups to work on, of `splits` that may have.
+int64_t used_splits(int64_t groups, int64_t splits) {
+  const int64_t each = (groups + splits - 1) / splits;
+  return (groups + each - 1) / each;
+}
+
 template <int F8, typename Tout, int TOK>
 cudaError_t launch_thin(const BlockMmParams& p, int64_t splits, bool& encoded, cudaStream_t st) {
   BlockMmMaps maps;
@@ -243,7 +249,7 @@ cudaError_t launch_thin(const BlockMmParams& p, int64_t splits, bool& encoded, c
   q.n = static_cast<int32_t>(p.n);
   q.groups = static_cast<int32_t>(groups);
   q.groups_per_split = static_cast<int32_t>((groups + splits - 1) / splits);
-  q.splits = (q.groups + q.groups_per_split - 1) / q.groups_per_split;  // none without a group
+  q.splits = static_cast<int32_t>(used_splits(groups, splits));
   q.own = (TOK + q.splits - 1) / q.splits;
   q.wide_stores = aligned(p.out, 16) && (p.out_stride * (int64_t)sizeof(Tout)) % 16 == 0;
   return launch_umma(block_mm_thin_kernel<F8, Tout, TOK>, dim3(static_cast<unsigned>(n_tiles * q.splits), static_cast<unsigned>(m_tiles)),
@@ -325,6 +331,21 @@ KVC_API int kvc_fp8_block_scaled_mm_clear_device_status(void) {
   if (e == cudaSuccess) e = cudaMemcpyToSymbol(kvc::g_block_mm_status, &zero, sizeof(int));
   if (e != cudaSuccess)
     return kvc::fail(KVC_ERR_CUDA, std::string("fp8_block_scaled_mm_clear_device_status: ") + cudaGetErrorString(e));
+  return KVC_OK;
+}
+
+KVC_API int kvc_fp8_block_scaled_mm_plan(int64_t m, int64_t n, int64_t k, int32_t* tile_tokens, int32_t* splits) {
+  using namespace kvc;
+  if (m < 1 || n < 1 || k < 1 || m > 0x3FFFFFFFll || n > 0x3FFFFFFFll || k > 0x3FFFFFFFll)
+    return fail(KVC_ERR_INVALID_ARG, "fp8_block_scaled_mm_plan: sizes out of range");
+  BlockMmParams p{};
+  p.m = m;
+  p.n = n;
+  p.k = k;
+  const MmPlan plan = plan_mm(p);
+  const int64_t groups = (k + kMmGroup - 1) / kMmGroup;
+  if (tile_tokens) *tile_tokens = plan.tokens > 0 ? plan.tokens : 256;
+  if (splits) *splits = static_cast<int32_t>(plan.tokens > 0 ? used_splits(groups, plan.splits) : 1);
   return KVC_OK;
 }
 

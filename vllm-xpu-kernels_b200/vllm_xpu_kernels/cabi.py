@@ -47,6 +47,7 @@ SYMBOLS = (
     "kvc_selftest_bounded_wait_gives_up",
     "kvc_dynamic_per_token_group_scaled_fp8_quant",
     "kvc_fp8_block_scaled_mm",
+    "kvc_fp8_block_scaled_mm_plan",
     "kvc_fp8_block_scaled_mm_device_status",
     "kvc_fp8_block_scaled_mm_clear_device_status",
     "kvc_fp8_block_scaled_mm_selftest_gives_up",
@@ -122,6 +123,8 @@ def lib() -> ctypes.CDLL:
         L.kvc_dynamic_per_token_group_scaled_fp8_quant.argtypes = [vp] * 4 + [i64] * 7 + [ci, ci, vp]
         L.kvc_fp8_block_scaled_mm.restype = ci
         L.kvc_fp8_block_scaled_mm.argtypes = [vp] * 5 + [i64] * 10 + [ci, ci, vp]
+        L.kvc_fp8_block_scaled_mm_plan.restype = ci
+        L.kvc_fp8_block_scaled_mm_plan.argtypes = [i64] * 3 + [ctypes.POINTER(ctypes.c_int32)] * 2
         L.kvc_fp8_block_scaled_mm_device_status.restype = ci
         L.kvc_fp8_block_scaled_mm_device_status.argtypes = [ctypes.POINTER(ci)]
         L.kvc_fp8_block_scaled_mm_clear_device_status.restype = ci
@@ -496,6 +499,13 @@ def fp8_block_scaled_mm(out, a, b, a_scales, b_scales, stream=None) -> None:
         out.data_ptr(), a.data_ptr(), b.data_ptr(), a_scales.data_ptr(), b_scales.data_ptr(), a.shape[0], b.shape[0],
         a.shape[1], out.stride(0), a.stride(0), b.stride(0), a_scales.stride(0), a_scales.stride(1), b_scales.stride(0),
         b_scales.stride(1), _in_dtype(out), FP8_CODE[a.dtype], _stream(stream)))
+
+
+def fp8_block_scaled_mm_plan(m: int, n: int, k: int) -> tuple[int, int]:
+    """``kvc_fp8_block_scaled_mm_plan``: (rows of a per tile, CTAs that divide a tile's groups) of that product."""
+    tokens, splits = ctypes.c_int32(0), ctypes.c_int32(0)
+    _check(lib().kvc_fp8_block_scaled_mm_plan(m, n, k, ctypes.byref(tokens), ctypes.byref(splits)))
+    return tokens.value, splits.value
 
 
 def fp8_block_scaled_mm_device_status() -> int:
