@@ -576,9 +576,9 @@ def _cache_list(caches, ref_counts=None):
     if not caches:
         return ptrs, 0, 0, 0, 1, 0, 0
     first = caches[0]
-    page = first[0].numel() * first.element_size()
+    page = first.shape[1:].numel() * first.element_size()
     for c in caches:
-        if (not c[0].is_contiguous() or c.shape[0] != first.shape[0] or c[0].numel() * c.element_size() != page
+        if (not c[:1].is_contiguous() or c.shape[0] != first.shape[0] or c.shape[1:].numel() * c.element_size() != page
                 or c.stride(0) * c.element_size() != first.stride(0) * first.element_size()):
             raise RuntimeError("caches must have dense pages of the same size")
     return ptrs, len(caches), first.shape[0], first.stride(0) * first.element_size(), 1, page, page
