@@ -421,6 +421,9 @@ KVC_API int kvc_multi_axis_rotary_embedding_and_cache_flash(
  *                     or that an earlier i names (with valid indices and a parent that is not empty, even where no page
  *                     was left for it), a parent longer than the table, or no page left.  Lengths and
  *                     tables of forks that were not made stay as they were.
+ *                     Entries of the parent's row that name no page (negative, or past the pool) are the child's too.  Where
+ *                     the last, partly filled page is such an entry the child still gets a page of its own, but nothing is
+ *                     copied into it: block_mapping[i] then holds that entry as its source.
  * kvc_free_blocks     for each of the sequences: lowers the counts of its pages, sets their table entries to -1 and its
  *                     length to 0.  Indices outside [0, num_seqs), empty rows and repetitions change nothing.
  * kvc_compact_blocks  with U pages in use: the k-th highest page in use at or above U moves to the k-th lowest free page,
