@@ -41,6 +41,10 @@ __device__ __forceinline__ bool mm_wait(uint64_t* bar, uint32_t parity, volatile
                                         uint32_t max_tries = umma::kMaxTries) {
   return __all_sync(0xFFFFFFFFu, umma::mbar_wait_bounded(bar, parity, abort_word, max_tries));
 }
+// The same for two events with one vote (a second one costs 0.08 us of 8.1 at 1 x 6144 x 4096).
+__device__ __forceinline__ bool mm_wait(uint64_t* bar, uint32_t parity, uint64_t* bar2, uint32_t parity2, volatile uint32_t* abort_word) {
+  return __all_sync(0xFFFFFFFFu, umma::mbar_wait_bounded(bar, parity, abort_word) && umma::mbar_wait_bounded(bar2, parity2, abort_word));
+}
 // A wait that ignores the abort word: lets what is in flight land before the CTA ends.
 __device__ __forceinline__ void mm_wait_limited(uint64_t* bar, uint32_t parity) {
   for (uint32_t i = 0; i < umma::kMaxTries; ++i)
@@ -320,8 +324,7 @@ __global__ void __launch_bounds__(ThinCfg<TOK>::kThreads, ThinCfg<TOK>::kCtasPer
     Ring<Cfg::kStages, kTakeTurns> at(warp - kMmaWarp);
     Ring<Cfg::kBuffers, kTakeTurns> buf(warp - kMmaWarp);
     for (int i = warp - kMmaWarp; i < count; i += kTakeTurns, at.advance(), buf.advance()) {
-      if (!mm_wait(taken + buf.slot, buf.parity ^ 1, abort_word)) break;
-      if (!mm_wait(full + at.slot, at.parity, abort_word)) break;
+      if (!mm_wait(taken + buf.slot, buf.parity ^ 1, full + at.slot, at.parity, abort_word)) break;
       fence_after_thread_sync();
       if (elect_one()) {
         const uint32_t base = smem_addr(smem + at.slot * Cfg::kStageBytes);
@@ -743,8 +746,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       const int mine = pair < tiles ? (tiles - 1 - pair) / pairs + 1 : 0;  // tiles of this pair
       const int64_t steps = static_cast<int64_t>(mine) * p.groups;
       for (int64_t it = me; it < steps; it += 2, at.advance(), parity ^= 1) {
-        if (!mm_wait(taken + me, parity ^ 1, abort_word)) break;
-        if (!mm_wait(full + at.slot, at.parity, abort_word)) break;
+        if (!mm_wait(taken + me, parity ^ 1, full + at.slot, at.parity, abort_word)) break;
         fence_after_thread_sync();
         if (elect_one()) {
           const uint32_t base = smem_addr(smem + at.slot * Cfg::kStageBytes);
