@@ -36,17 +36,19 @@ def test_no_cta_is_written_before_it_has_begun():
 def test_nothing_is_in_flight_when_memory_is_given_back():
     """A wait can give up in any warp until the last barrier, so only behind it is it known whether copies and MMAs may still be
     under way; they are waited for there, before the tensor memory is freed and the CTA ends."""
-    for name, barrier, free in (("block_mm_thin_kernel", "__syncthreads()", "tmem_dealloc("),
-                                ("block_mm_wide_kernel", "cluster_sync()", "tmem_dealloc_pair(")):
+    for name, barriers, free in (("block_mm_thin_kernel", ("__syncthreads()", "__syncthreads()"), "tmem_dealloc("),
+                                 ("block_mm_wide_kernel", ("cluster_sync()", "mm_wait_limited(drained"), "tmem_dealloc_pair(")):
         body = kernel(name)
         drain, end = body.rindex("if (*abort_word) {"), body.index(free)
-        # behind the last wait that can give up and a barrier of everyone, and with another such barrier before the memory goes
+        # behind the last wait that can give up and a barrier of everyone; and everyone who frees memory or ends last waits for it
         last_wait = max(m.end() for m in re.finditer(r"\b(mm_wait|mbar_wait_bounded)\(", body))
-        assert last_wait < body.rindex(barrier, 0, drain) < drain < body.rindex(barrier, 0, end) < end
+        assert last_wait < body.rindex(barriers[0], 0, drain) < drain < body.rindex(barriers[1], 0, end) < end
         drains = [m.start() for m in re.finditer(r"\bmm_wait_limited\(", body)]
         assert len(drains) == 2 and all(drain < d < end for d in drains)
         commit = re.search(r"mma_commit(_pair)?\(drained\)", body)
         assert drain < commit.start() < drains[1]
+    # the pair: one arrival for the copies and one of each issuing warp
+    assert "mbar_init(drained, 3)" in kernel("block_mm_wide_kernel") and "mbar_init(drained, Cfg::kIssuers)" in kernel("block_mm_thin_kernel")
 
 
 def test_lanes_leave_a_loop_together():
@@ -71,7 +73,7 @@ def test_results_that_could_not_be_computed_are_nan():
     stores = [m.group(0) for m in re.finditer(r"from_f32<Tout>\([^;]*;|store_words<Tout, 32>\([^;]*;", thin[look:])]
     assert len(stores) == 2 and all("lost ? " in s for s in stores)
     wide = kernel("block_mm_wide_kernel")
-    look = wide.index("if (*abort_word) {")
-    epilogue = wide.index("setmaxnreg.inc")
-    waits = [m.end() for m in re.finditer(r"\b(mm_wait|mbar_wait_bounded)\(", wide[epilogue:])]
-    assert epilogue + max(waits) < look < wide.index("store_chunk(") < wide.index("st_if(")
+    additions = wide[wide.index("if (warp < 8) {"):wide.index("setmaxnreg.dec")]
+    look = additions.index("if (*abort_word) {")
+    waits = [m.end() for m in re.finditer(r"\b(mm_wait|mbar_wait_bounded)\(", additions)]
+    assert len(waits) == 2 and max(waits) < look < additions.index("store_chunk(") < additions.index("st_if(")

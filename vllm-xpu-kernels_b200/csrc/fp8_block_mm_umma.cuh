@@ -622,6 +622,9 @@ __device__ __forceinline__ void wide_tma_load(uint32_t dst, const CUtensorMap* m
       : "memory");
 }
 
+// By every thread of the CTA, from wherever its role ends.
+__device__ __forceinline__ void wide_cta_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWideThreads) : "memory"); }
+
 template <int F8, typename Tout>
 __global__ void __launch_bounds__(kWideThreads, 1)
     block_mm_wide_kernel(const __grid_constant__ BlockMmMaps maps, const __grid_constant__ WideParams p) {
@@ -639,7 +642,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   uint64_t* drained = used + Cfg::kScaleSlots;     // after a wait that gave up: no MMA of the pair is in flight
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::kBars);
   volatile uint32_t* abort_word = tmem_slot + 1;
-  volatile uint32_t* peer_asked = tmem_slot + 2;   // the even CTA's: groups that the odd one has asked for
+  // words 2 and 3 behind it, of the even CTA: groups that its own and the odd CTA's loading warp have asked for
   float4* scales = reinterpret_cast<float4*>(smem + Cfg::kOffScales);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
@@ -659,7 +662,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       mbar_init(scaled + i, 1);
       mbar_init(used + i, 8);
     }
-    mbar_init(drained, 2);
+    mbar_init(drained, 3);
     *abort_word = 0;
     mbar_init_fence();
   }
@@ -673,93 +676,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   const uint32_t tmem = *tmem_slot;
   const int tiles = p.m_tiles * p.n_tiles;
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  uint32_t asked = 0;  // groups that the loading warp has asked for
 
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideOtherRegs));
-    if (warp == 10) {
-      Ring<Cfg::kStages> at;
-      bool ok = true;
-      for (int tile = pair; ok && tile < tiles; tile += pairs) {
-        int mt, nt;
-        wide_tile(p, tile, mt, nt);
-        const int m0 = mt * 256 + rank * 128, n0 = nt * 256 + rank * 128;
-        for (int g = 0; g < p.groups; ++g, ++asked, at.advance()) {
-          ok = mm_wait(empty + at.slot, at.parity ^ 1, abort_word);
-          if (!ok) break;
-          if (elect_one()) {
-            if (rank == 0) mm_expect_tx(full + at.slot, 2 * Cfg::kStageBytes);
-            const uint32_t bar = cluster_addr(smem_addr(full + at.slot), 0);
-            const uint32_t dst = smem_addr(smem + at.slot * Cfg::kStageBytes);
-            wide_tma_load(dst, &maps.a, bar, g * 128, m0);
-            wide_tma_load(dst + Cfg::kTile, &maps.b, bar, g * 128, n0);
-          }
-          __syncwarp();
-        }
-      }
-    } else if (warp == 11) {
-      Ring<Cfg::kScaleSlots> at;
-      bool ok = true;
-      for (int tile = pair; ok && tile < tiles; tile += pairs) {
-        int mt, nt;
-        wide_tile(p, tile, mt, nt);
-        // rows and column blocks past the end repeat the last one: their products are not stored
-        const int last = (p.n - 1) / 128;
-        const float* sb0 = p.b_scales + min(nt * 2, last) * p.bs_stride_n;
-        const float* sb1 = p.b_scales + min(nt * 2 + 1, last) * p.bs_stride_n;
-        for (int g = 0; g < p.groups; g += Cfg::kScaleGroups, at.advance()) {
-          ok = mm_wait(used + at.slot, at.parity ^ 1, abort_word);
-          if (!ok) break;
-          const int m = mt * 256 + static_cast<int>(rank) * 128 + lane;
-          float vb[2][4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            vb[0][k] = g + k < p.groups ? ld_ahead(sb0 + (g + k) * p.bs_stride_g) : 0.0f;
-            vb[1][k] = g + k < p.groups ? ld_ahead(sb1 + (g + k) * p.bs_stride_g) : 0.0f;
-          }
-#pragma unroll 1
-          for (int r = 0; r < 4; r += 2) {  // two rows a lane at a time
-            float va[2][4];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float* sa = p.a_scales + min(m + (r + i) * 32, p.m - 1) * p.as_stride_m + g * p.as_stride_g;
-#pragma unroll
-              for (int k = 0; k < 4; ++k) va[i][k] = g + k < p.groups ? ld_ahead(sa + k * p.as_stride_g) : 0.0f;
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int i = 0; i < 2; ++i)
-                scales[at.slot * 256 + h * 128 + (r + i) * 32 + lane] =
-                    make_float4(__fmul_rn(va[i][0], vb[h][0]), __fmul_rn(va[i][1], vb[h][1]),
-                                __fmul_rn(va[i][2], vb[h][2]), __fmul_rn(va[i][3], vb[h][3]));
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(scaled + at.slot);
-        }
-      }
-    } else if (rank == 0) {
-      constexpr uint32_t idesc = instr_desc_f8(256, 256, F8 == KVC_KV_FP8_E5M2);
-      const int me = warp - 8;
-      Ring<Cfg::kStages, 2> at(me);
-      uint32_t parity = 0;  // of buffer `me`, the only one this warp uses
-      const int mine = pair < tiles ? (tiles - 1 - pair) / pairs + 1 : 0;  // tiles of this pair
-      const int64_t steps = static_cast<int64_t>(mine) * p.groups;
-      for (int64_t it = me; it < steps; it += 2, at.advance(), parity ^= 1) {
-        if (!mm_wait(taken + me, parity ^ 1, full + at.slot, at.parity, abort_word)) break;
-        fence_after_thread_sync();
-        if (elect_one()) {
-          const uint32_t base = smem_addr(smem + at.slot * Cfg::kStageBytes);
-          const uint64_t da = smem_desc_sw128(base, 0, 1024), db = smem_desc_sw128(base + Cfg::kTile, 0, 1024);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) mma_f8_ss_pair(tmem + me * 256, da + 2 * k, db + 2 * k, idesc, k > 0);
-          mma_commit_pair(empty + at.slot);
-          mma_commit_pair(ready + me);
-        }
-        __syncwarp();
-      }
-    }
-  } else {
+  if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWideEpilogueRegs));
     const int half = warp >> 2, row = threadIdx.x & 127;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + half * 128;
@@ -892,31 +810,127 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         }
       }
     }
-  }
-  __syncwarp();
-  // the CTAs of a pair give up together: copies and MMAs of either touch barriers or memory of the other
-  if (*abort_word) st_cluster(cluster_addr(smem_addr(tmem_slot + 1), rank ^ 1), 1);
-  if (rank == 1 && warp == 10 && lane == 0) st_cluster(cluster_addr(smem_addr(tmem_slot + 2), 0), asked);
-  __syncwarp();
-  fence_before_thread_sync();
-  cluster_sync();  // the even CTA's MMAs read the odd one's shared memory, and barriers are signalled across
-  fence_after_thread_sync();
-  if (*abort_word) {  // final by now, and the same in both
-    if (rank == 0 && warp == 10) {  // both CTAs' copies count on the even one's barriers
-      const uint32_t end = max(asked, *peer_asked);
-      for (uint32_t i = end > Cfg::kStages ? end - Cfg::kStages : 0; i < end; ++i)
-        mm_wait_limited(full + i % Cfg::kStages, (i / Cfg::kStages) & 1);
-    } else if (warp == 8 || warp == 9) {
-      if (rank == 0 && elect_one()) mma_commit_pair(drained);
-      mm_wait_limited(drained, 0);
-    }
+    // This role ends here, not where the others meet: any code behind a meeting point of all of them cost its loop time
+    // (zero operands: 994 us this way, otherwise 1006 to 1042 with what stands below).
     __syncwarp();
     fence_before_thread_sync();
+    wide_cta_sync();
     cluster_sync();
+    return;
+  }
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideOtherRegs));
+  if (warp == 10) {
+    Ring<Cfg::kStages> at;
+    bool ok = true;
+    uint32_t asked = 0;
+    for (int tile = pair; ok && tile < tiles; tile += pairs) {
+      int mt, nt;
+      wide_tile(p, tile, mt, nt);
+      const int m0 = mt * 256 + rank * 128, n0 = nt * 256 + rank * 128;
+      for (int g = 0; g < p.groups; ++g, ++asked, at.advance()) {
+        ok = mm_wait(empty + at.slot, at.parity ^ 1, abort_word);
+        if (!ok) break;
+        if (elect_one()) {
+          if (rank == 0) mm_expect_tx(full + at.slot, 2 * Cfg::kStageBytes);
+          const uint32_t bar = cluster_addr(smem_addr(full + at.slot), 0);
+          const uint32_t dst = smem_addr(smem + at.slot * Cfg::kStageBytes);
+          wide_tma_load(dst, &maps.a, bar, g * 128, m0);
+          wide_tma_load(dst + Cfg::kTile, &maps.b, bar, g * 128, n0);
+        }
+        __syncwarp();
+      }
+    }
+    if (lane == 0) st_cluster(cluster_addr(smem_addr(tmem_slot + 2 + rank), 0), asked);
+  } else if (warp == 11) {
+    Ring<Cfg::kScaleSlots> at;
+    bool ok = true;
+    for (int tile = pair; ok && tile < tiles; tile += pairs) {
+      int mt, nt;
+      wide_tile(p, tile, mt, nt);
+      // rows and column blocks past the end repeat the last one: their products are not stored
+      const int last = (p.n - 1) / 128;
+      const float* sb0 = p.b_scales + min(nt * 2, last) * p.bs_stride_n;
+      const float* sb1 = p.b_scales + min(nt * 2 + 1, last) * p.bs_stride_n;
+      for (int g = 0; g < p.groups; g += Cfg::kScaleGroups, at.advance()) {
+        ok = mm_wait(used + at.slot, at.parity ^ 1, abort_word);
+        if (!ok) break;
+        const int m = mt * 256 + static_cast<int>(rank) * 128 + lane;
+        float vb[2][4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          vb[0][k] = g + k < p.groups ? ld_ahead(sb0 + (g + k) * p.bs_stride_g) : 0.0f;
+          vb[1][k] = g + k < p.groups ? ld_ahead(sb1 + (g + k) * p.bs_stride_g) : 0.0f;
+        }
+#pragma unroll 1
+        for (int r = 0; r < 4; r += 2) {  // two rows a lane at a time
+          float va[2][4];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float* sa = p.a_scales + min(m + (r + i) * 32, p.m - 1) * p.as_stride_m + g * p.as_stride_g;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) va[i][k] = g + k < p.groups ? ld_ahead(sa + k * p.as_stride_g) : 0.0f;
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              scales[at.slot * 256 + h * 128 + (r + i) * 32 + lane] =
+                  make_float4(__fmul_rn(va[i][0], vb[h][0]), __fmul_rn(va[i][1], vb[h][1]),
+                              __fmul_rn(va[i][2], vb[h][2]), __fmul_rn(va[i][3], vb[h][3]));
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(scaled + at.slot);
+      }
+    }
+  } else if (rank == 0) {
+    constexpr uint32_t idesc = instr_desc_f8(256, 256, F8 == KVC_KV_FP8_E5M2);
+    const int me = warp - 8;
+    Ring<Cfg::kStages, 2> at(me);
+    uint32_t parity = 0;  // of buffer `me`, the only one this warp uses
+    const int mine = pair < tiles ? (tiles - 1 - pair) / pairs + 1 : 0;  // tiles of this pair
+    const int64_t steps = static_cast<int64_t>(mine) * p.groups;
+    for (int64_t it = me; it < steps; it += 2, at.advance(), parity ^= 1) {
+      if (!mm_wait(taken + me, parity ^ 1, full + at.slot, at.parity, abort_word)) break;
+      fence_after_thread_sync();
+      if (elect_one()) {
+        const uint32_t base = smem_addr(smem + at.slot * Cfg::kStageBytes);
+        const uint64_t da = smem_desc_sw128(base, 0, 1024), db = smem_desc_sw128(base + Cfg::kTile, 0, 1024);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mma_f8_ss_pair(tmem + me * 256, da + 2 * k, db + 2 * k, idesc, k > 0);
+        mma_commit_pair(empty + at.slot);
+        mma_commit_pair(ready + me);
+      }
+      __syncwarp();
+    }
+  }
+  __syncwarp();
+  fence_before_thread_sync();
+  wide_cta_sync();
+  if (warp == 8) {  // no warp of this CTA can give up any more; the CTAs of a pair do so together
+    if (*abort_word) st_cluster(cluster_addr(smem_addr(tmem_slot + 1), rank ^ 1), 1);
+    __syncwarp();
+  }
+  cluster_sync();  // the even CTA's MMAs read the odd one's shared memory, and barriers are signalled across
+  fence_after_thread_sync();
+  if (*abort_word) {  // the same in both
+    if (rank == 0 && warp == 10) {  // both CTAs' copies count on the even one's barriers
+      const volatile uint32_t* asked = tmem_slot + 2;
+      const uint32_t end = max(asked[0], asked[1]);
+      for (uint32_t i = end > Cfg::kStages ? end - Cfg::kStages : 0; i < end; ++i)
+        mm_wait_limited(full + i % Cfg::kStages, (i / Cfg::kStages) & 1);
+      __syncwarp();
+      if (lane < 2)
+        asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr(smem_addr(drained), lane)) : "memory");
+    } else if (rank == 0 && warp < 10) {
+      if (elect_one()) mma_commit_pair(drained);
+    }
+    __syncwarp();
+    mm_wait_limited(drained, 0);  // neither CTA ends, or gives memory back, before
     fence_after_thread_sync();
   }
+  __syncwarp();
   if (warp == 8) tmem_dealloc_pair(tmem, 512);
-  if (threadIdx.x == 0 && *abort_word) atomicMax(&g_block_mm_status, 1);
+  if (warp == 11 && lane == 0 && *abort_word) atomicMax(&g_block_mm_status, 1);
 }
 
 // Self-test of what a CTA does when a wait gives up: one warp waits, with a limit of `tries` tries (about 20 us each), for an
