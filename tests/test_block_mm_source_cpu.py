@@ -47,6 +47,8 @@ def test_nothing_is_in_flight_when_memory_is_given_back():
         assert len(drains) == 2 and all(drain < d < end for d in drains)
         commit = re.search(r"mma_commit(_pair)?\(drained\)", body)
         assert drain < commit.start() < drains[1]
+    # whoever waits for the pair's drain has more patience than the drain's own waits, one per stage, can take together
+    assert "mm_wait_limited(drained, 0, Cfg::kStages + 2)" in kernel("block_mm_wide_kernel")
     # the pair: one arrival for the copies and one of each issuing warp
     assert "mbar_init(drained, 3)" in kernel("block_mm_wide_kernel") and "mbar_init(drained, Cfg::kIssuers)" in kernel("block_mm_thin_kernel")
 
